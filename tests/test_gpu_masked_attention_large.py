@@ -1,0 +1,94 @@
+"""Masked attention where calls are large enough for two row tiles a block (from two row tiles an SM
+on), against a plain 64-bit implementation on the GPU.
+
+Tolerances are those of the small cases, whose derivation does not look at sizes: 2 roundings of
+2^-9 for out, 3 for a gradient, and for a row eight times as much of the larger of its own and
+the mean row's norm."""
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_masked_attention import DEV, TOL_GRAD, TOL_OUT, close, inputs
+from xfold_cpu_b200 import _capi, native
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    _capi.device_error(clear=True)
+    yield
+    torch.cuda.synchronize()
+    assert _capi.device_error(clear=True) == 0
+
+
+def reference(q, k, v, dout=None, softcap=0.0, slopes=None, causal=False, prefix=None,
+              documents=None):
+    """(out[, dq, dk, dv]) in 64 bits, a row of the batch at a time."""
+    B, H, nq, d = q.shape
+    G, nk = k.shape[1:3]
+    rep = H // G
+    pos, key = torch.arange(nq, device=DEV) + nk - nq, torch.arange(nk, device=DEV)
+    results = []
+    for b in range(B):
+        vis = torch.ones(nq, nk, dtype=torch.bool, device=DEV)
+        if causal:
+            vis = key[None] <= pos[:, None]
+            if prefix is not None:
+                vis = vis | (key < prefix[b])[None]
+        if documents is not None:
+            qd, kd = (x.expand(B, -1)[b] for x in documents)
+            vis = vis & (qd[:, None] == kd[None]) & (kd >= 0)[None]
+        some, seen = vis.any(1), vis.any(0)
+        # what no query sees, or sees nothing, may hold anything
+        qq = torch.where(some[:, None], q[b].double(), 0.0)
+        kk, vv = (torch.where(seen[:, None], t[b].double(), 0.0).repeat_interleave(rep, 0)
+                  for t in (k, v))
+        x = d ** -0.5 * (qq @ kk.transpose(-1, -2))
+        t = torch.tanh(x / softcap) if softcap else None
+        s = softcap * t if softcap else x
+        if slopes is not None:
+            s = s - slopes.double()[:, None, None] * (pos[:, None] - key[None]).abs()
+        s = s.masked_fill(~vis, -math.inf).masked_fill(~some[:, None], 0.0)
+        p = torch.softmax(s, -1).masked_fill(~vis, 0.0)
+        out = p @ vv
+        row = [out]
+        if dout is not None:
+            do = torch.where(some[:, None], dout[b].double(), 0.0)
+            dx = p * (do @ vv.transpose(-1, -2) - (do * out).sum(-1, keepdim=True)) * d ** -0.5
+            if softcap:
+                dx = dx * (1 - t * t)
+            row += [dx @ kk, (dx.transpose(-1, -2) @ qq).view(G, rep, nk, d).sum(1),
+                    (p.transpose(-1, -2) @ do).view(G, rep, nk, d).sum(1)]
+        results.append([r.cpu() for r in row])
+    return [torch.stack(r) for r in zip(*results)]
+
+
+def two_row_tiles_a_block(q, k):
+    rep = q.shape[1] // k.shape[1]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    return q.shape[0] * k.shape[1] * -(-q.shape[2] // (128 // rep)) >= 2 * sms
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("d", [64, 128])
+def test_padding_among_the_keys_of_a_block_s_second_tile(d, bad):
+    """The second row tile of each block sees none of the first tile's keys, so its list starts
+    seven key tiles after the block's; V of its padded keys holds NaN or infinities."""
+    H, nq, nk, cut = 80, 256, 903, 7 * 64
+    q, k, v, _ = inputs(2, H, H, nq, nk, d, BF16)
+    assert two_row_tiles_a_block(q, k)
+    q_ids = (torch.arange(nq, device=DEV) >= 128).int()[None]
+    k_ids = (torch.arange(nk, device=DEV) >= cut).int().expand(2, nk).clone()
+    g = torch.Generator().manual_seed(7)
+    k_ids[(torch.rand(2, nk, generator=g) < 0.3).to(DEV)] = -1
+    for t in (k, v):
+        t.masked_fill_((k_ids < 0)[:, None, :, None], bad)
+    ref, = reference(q, k, v, documents=(q_ids, k_ids))
+    for save in (False, True):
+        got = native.masked_attention(q, k, v, documents=(q_ids, k_ids), save=save)
+        close(got[0] if save else got, ref, TOL_OUT[BF16], f"out, save={save}")
