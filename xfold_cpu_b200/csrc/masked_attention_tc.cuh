@@ -169,29 +169,6 @@ __device__ __forceinline__ void mt_zero_row(uint8_t* tile, int row) {
       reinterpret_cast<uint4*>(tile + c * (ROWS * 128) + row * 128)[e] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// Which of the 64 keys from key0 on are in no document, a bit each: one warp.
-__device__ __forceinline__ uint2 mt_padded_keys(const MaskedArgs& a, int b, int key0, bool any) {
-  if (!any) return make_uint2(0u, 0u);
-  const int32_t* kdoc = a.kdoc + b * a.kdoc_sb + key0 + (threadIdx.x & 31);
-  return make_uint2(__ballot_sync(0xffffffffu, kdoc[0] < 0),
-                    __ballot_sync(0xffffffffu, kdoc[32] < 0));
-}
-// Zeros those rows of a loaded V tile, whatever their memory holds.  The warp that issues
-// the products does it: it alone waits for every load of a stage in turn, so that a wait cannot
-// pass on the phase of the stage's last tile, and no other warp's order matters.
-template <int DP>
-__device__ __forceinline__ void mt_zero_keys(uint8_t* tile, uint2 padded) {
-  // 16-byte pieces, eight to a 128-byte row, 64 rows to a chunk of 64 dims
-#pragma unroll 4
-  for (int x = threadIdx.x & 31; x < kMtKeys * DP / 8; x += 32) {
-    const int row = (x >> 3) & (kMtKeys - 1);
-    if (((row < 32 ? padded.x : padded.y) >> (row & 31)) & 1u)
-      reinterpret_cast<uint4*>(tile)[x] = make_uint4(0u, 0u, 0u, 0u);
-  }
-  fence_async_smem();
-  __syncwarp();
-}
-
 // After a wait that gave up: time for the loads in flight to land before the block exits.
 __device__ __forceinline__ void mt_drain(volatile int* abort_flag) {
   if (!*abort_flag) return;
@@ -472,7 +449,12 @@ __global__ void __launch_bounds__(MtForward<DP, SLOTS_>::kThreads, 1)
       int st = 0;
       uint32_t ph = 1;
       for (int n = 0; n < count; ++n) {
-        const int key0 = (tile0 + (all_tiles[n] & kMtTile)) * kMtKeys;
+        const uint32_t entry = all_tiles[n];
+        const int key0 = (tile0 + (entry & kMtTile)) * kMtKeys;
+        // The softmax warps wait for V of a padded tile, but not for every tile's, so their wait
+        // could pass on the phase of the stage's last tile.  K, and with it S, of a padded tile
+        // comes after that tile's V has been used.
+        if ((entry & kMtPadded) && !mbar_wait(&v_empty[st], ph, kErrWaitProducer, abort_flag)) break;
         if (!mbar_wait(&k_empty[st], ph, kErrWaitProducer, abort_flag)) break;
         mbar_arrive_expect_tx(&k_full[st], L::kTile);
         mt_load_keys<DP, kMtKeys>(sK + st * L::kTile, &tmK, &k_full[st], key0, g * mk.head, b * mk.batch);
@@ -524,10 +506,7 @@ __global__ void __launch_bounds__(MtForward<DP, SLOTS_>::kThreads, 1)
       bool ok = true;
       for (int n = 0; ok && n < count; ++n) {
         const uint32_t entry = all_tiles[n];
-        const uint2 padded = mt_padded_keys(a, b, (tile0 + (entry & kMtTile)) * kMtKeys,
-                                            (entry & kMtPadded) != 0);
         ok = mbar_wait(&v_full[st], ph, kErrWaitMma, abort_flag);
-        if (ok && (padded.x | padded.y)) mt_zero_keys<DP>(sV + st * L::kTile, padded);
         const uint32_t v_addr = smem_u32(sV + st * L::kTile);
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
@@ -688,6 +667,16 @@ __global__ void __launch_bounds__(MtForward<DP, SLOTS_>::kThreads, 1)
         }
       }
       tmem_wait_st();
+      }
+      // ---- V rows of keys in no document become zeros, whatever their memory holds
+      if (entry & kMtPadded) {
+        int n = m;  // the tile's place among the block's: its stage
+        while ((all_tiles[n] & kMtTile) != (entry & kMtTile)) ++n;
+        ok = mbar_wait(&v_full[n % NS], (n / NS) & 1, kErrWaitSoftmax, abort_flag);
+        if (!ok) break;
+        if (row < kMtKeys && a.kdoc[b * a.kdoc_sb + key0 - col0 + row] < 0)
+          mt_zero_row<DP, kMtKeys>(sV + (n % NS) * L::kTile, row);
+        fence_async_smem();
       }
       tc_fence_before();
       mbar_arrive(&p_full[NB * s + buf]);
