@@ -92,3 +92,16 @@ def test_padding_among_the_keys_of_a_block_s_second_tile(d, bad):
     for save in (False, True):
         got = native.masked_attention(q, k, v, documents=(q_ids, k_ids), save=save)
         close(got[0] if save else got, ref, TOL_OUT[BF16], f"out, save={save}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tiles", range(1, 8))
+def test_every_last_buffer(d, tiles):
+    """Two groups of warps take a row tile's key tiles in turn; the last is the one's or the
+    other's, in a buffer's first or a later use."""
+    q, k, v, _ = inputs(2, 80, 80, 256, 64 * tiles - 5, d, BF16)
+    assert two_row_tiles_a_block(q, k)
+    ref, = reference(q, k, v)
+    for save in (False, True):
+        got = native.masked_attention(q, k, v, save=save)
+        close(got[0] if save else got, ref, TOL_OUT[BF16], f"out, save={save}")

@@ -683,11 +683,15 @@ __global__ void __launch_bounds__(MtForward<DP, SLOTS_>::kThreads, 1)
     }
     const int m = count - 1;
     // ---- results: the halves' l on the last m, then half of the columns each
+    // Both halves are done with the rows' m.  The half that did not take the last tile has not
+    // seen its buffer's last phase, which the other half's scores came after: it waits behind it.
+    tc_fence_before();
+    named_barrier(1 + s, 256);
+    tc_fence_after();
     if (m >= 0 && ok) {
       ok = mbar_wait(&pv_done[NB * s + m % NB], (m / NB) & 1, kErrWaitSoftmax, abort_flag);
       tc_fence_after();
     }
-    named_barrier(1 + s, 256);  // both halves are done with the rows' m
     if (m >= 0) {
       const float m_end = row_m[s * 128 + row];
       l *= m_end == m_ref || m_end == -INFINITY ? 1.f : ex2_approx(m_ref - m_end);
