@@ -38,8 +38,19 @@ class PackedAttention(nn.Module):
         self.output = nn.Parameter(torch.randn(c, h * d) * (h * d) ** -0.5)
         self.register_buffer("frequencies", native.rotary_frequencies(
             d if rotated is None else rotated, stretch=stretch), persistent=False)
-        slopes = torch.tensor([2.0 ** (-8.0 * (i + 1) / h) for i in range(h)]) if distance else None
+        slopes = torch.tensor([2.0 ** (-8.0 * (i + 1) / h) for i in range(h)],
+                              dtype=torch.float32) if distance else None
         self.register_buffer("slopes", slopes, persistent=False)
+
+    def _apply(self, fn, recurse: bool = True):
+        """Moves and casts the layer, but keeps frequencies and slopes in float32: an angle is
+        position * frequency, and 8 bits of a frequency are a turn off after some thousand tokens."""
+        kept = {name: t for name, t in self._buffers.items() if t is not None}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
 
     def _heads(self, x: torch.Tensor, positions, offset: int):
         """q [B, H, N, D], k and v [B, G, N, D] as views of one projection, q and k rotated."""
