@@ -1069,13 +1069,19 @@ def _strided(t: torch.Tensor) -> tuple[int, int, int, int]:
     return t.data_ptr(), s[0], s[1], s[2]
 
 
+def _integers(what: str, t: torch.Tensor) -> torch.Tensor:
+    """Integers in a type that keeps every value: int32 where it does, else int64."""
+    if t.dtype == torch.int32 or t.dtype == torch.int64:
+        return t
+    if t.is_floating_point() or t.is_complex() or t.dtype in (torch.bool, torch.uint64):
+        raise ValueError(f"{what} must be integers of at most 64 bits with a sign")
+    return t.to(torch.int64 if t.dtype == torch.uint32 else torch.int32)
+
+
 def _token_ints(what: str, t: torch.Tensor, B: int, n: int) -> tuple[torch.Tensor, int]:
     """int32 [n] or [B, n] with neighbouring tokens next to each other, and its batch stride
     (0 where one row serves the batch)."""
-    if t.dtype != torch.int32:
-        if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-            raise ValueError(f"{what} must be integers")
-        t = t.to(torch.int32)
+    t = _integers(what, t).to(torch.int32)
     shape = t.shape
     if shape != (B, n) and shape != (n,) and shape != (1, n):
         raise ValueError(f"{what} must be [{n}] or [{B}, {n}], got {list(shape)}")
@@ -1106,6 +1112,9 @@ def _masked_attention_args(q, k, v, scale, softcap, slopes, causal, prefix, docu
     if prefix is not None:
         if prefix.shape != (B,):
             raise ValueError(f"prefix must be [{B}], got {list(prefix.shape)}")
+        prefix = _integers("prefix", prefix)
+        if prefix.dtype != torch.int32:  # no row is longer than 2^30
+            prefix = prefix.clamp(0, 1 << 30)
         prefix = _token_ints("prefix", prefix, 1, B)[0]
         prefix_at = prefix.data_ptr()
     if q_doc is not None:
