@@ -715,7 +715,7 @@ XFB_API int xfb_layer_norm_backward(const void* dy, int64_t lddy, const void* x,
  * first `rotated` (even) dims turn in pairs, the others are copied.  Pair p of the token at
  * position t turns by t * frequencies[p] and grows by `magnitude`; pairs are the halves'
  * (p, p + rotated / 2), or neighbours (2p, 2p + 1) with `interleaved`.  positions[b][i]
- * (batch stride positions_sb), or `offset` + i where NULL.  inverse = 1 turns back: with
+ * (batch stride positions_sb; int64 with positions_64, else int32), or `offset` + i where NULL.  inverse = 1 turns back: with
  * the same magnitude it is the gradient of the forward call. */
 typedef struct xfb_rotary_args {
   const void* q;
@@ -727,11 +727,11 @@ typedef struct xfb_rotary_args {
   void* k_out;
   int64_t ko_sb, ko_sh, ko_sn;
   const float* frequencies;
-  const int32_t* positions;
+  const void* positions;
   int64_t positions_sb, offset;
   int64_t batch, heads, kv_heads, n, d, rotated;
   double magnitude;
-  int dtype, interleaved, inverse;
+  int dtype, interleaved, inverse, positions_64;
 } xfb_rotary_args;
 XFB_API int xfb_rotary(const xfb_rotary_args* args, void* stream);
 

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from test_gpu_masked_attention import DEV, check, inputs
+from test_gpu_rotary import reference as rotary_reference
 from xfold_cpu_b200 import native
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +33,23 @@ def test_unsigned_and_short_types():
     with pytest.raises(ValueError):
         native.masked_attention(q, k, v, causal=True,
                                 prefix=torch.zeros(2, dtype=torch.uint64, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_positions(dtype, interleaved):
+    """Positions around 2^32 and below zero.  An angle of 2^33 has a rounding of 2^-53 of it in the
+    reference and two in the kernel, 3e-6, beside the small positions' 1e-6 (f32) or 2^-9."""
+    q, k = (t[0] for t in (inputs(2, 3, 1, 40, 40, 64, dtype)[:1], inputs(2, 1, 1, 40, 40, 64, dtype)[:1]))
+    freq = native.rotary_frequencies(48).to(DEV)
+    positions = torch.arange(40).expand(2, 40) * 107_000_003 + torch.tensor([[1 << 31], [-(1 << 32)]])
+    got = native.rotary(q, k, freq, positions=positions.to(DEV), interleaved=interleaved)
+    tol = 4e-6 + (2.0 ** -9 if dtype == torch.bfloat16 else 0.0)
+    for x, y in zip((q, k), got):
+        ref = rotary_reference(x, freq, positions, interleaved, 1.0)
+        assert (y.cpu().double() - ref).norm().item() <= tol * ref.norm().item()
+    small = torch.arange(40, device=DEV) * 7
+    for other in (torch.int16, torch.int64, torch.uint32):
+        a = native.rotary(q, k, freq, positions=small.to(other), interleaved=interleaved)
+        b = native.rotary(q, k, freq, positions=small.int(), interleaved=interleaved)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

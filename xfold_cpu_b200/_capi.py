@@ -188,7 +188,7 @@ class RotaryArgs(ctypes.Structure):
     _fields_ = _fields("q:p q_sb:l q_sh:l q_sn:l k:p k_sb:l k_sh:l k_sn:l q_out:p qo_sb:l qo_sh:l "
                        "qo_sn:l k_out:p ko_sb:l ko_sh:l ko_sn:l frequencies:p positions:p "
                        "positions_sb:l offset:l batch:l heads:l kv_heads:l n:l d:l rotated:l "
-                       "magnitude:d dtype:i interleaved:i inverse:i")
+                       "magnitude:d dtype:i interleaved:i inverse:i positions_64:i")
 
 
 class MaskedAttentionArgs(ctypes.Structure):

@@ -34,7 +34,8 @@ struct RotaryArgs {
   int64_t B, n;
   int d, rotated;
   const float* freq;         // [rotated / 2]
-  const int32_t* positions;  // positions[b * pos_sb + i], or null: offset + i
+  const void* positions;     // positions[b * pos_sb + i], or null: offset + i
+  int positions_64;          // they are int64 (else int32)
   int64_t pos_sb;
   int64_t offset;
   float magnitude;
@@ -73,8 +74,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
     constexpr int PAIRS = INTERLEAVED ? (kPair ? 1 : VEC / 2) : VEC;
     float sn[PAIRS], cs[PAIRS];
     if (turns) {
-      const double position = a.positions ? static_cast<double>(a.positions[b * a.pos_sb + i])
-                                          : static_cast<double>(a.offset + i);
+      const int64_t place = b * a.pos_sb + i;
+      const double position = static_cast<double>(
+          a.positions == nullptr ? a.offset + i
+          : a.positions_64       ? static_cast<const int64_t*>(a.positions)[place]
+                                 : static_cast<const int32_t*>(a.positions)[place]);
 #pragma unroll
       for (int p = 0; p < PAIRS; ++p)
         rotary_sincos(position, a.freq[(INTERLEAVED ? dim / 2 : dim) + p], a.magnitude, a.inverse,

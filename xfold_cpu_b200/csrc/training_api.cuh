@@ -336,6 +336,7 @@ XFB_API int xfb_rotary(const xfb_rotary_args* args, void* stream) {
     r.rotated = static_cast<int>(a.rotated);
     r.freq = a.frequencies;
     r.positions = a.positions;
+    r.positions_64 = a.positions_64;
     r.pos_sb = a.positions_sb;
     r.offset = a.offset;
     r.magnitude = static_cast<float>(a.magnitude);

@@ -1023,10 +1023,10 @@ def _rotary(q, k, frequencies, positions, offset, interleaved, magnitude, invers
     if frequencies.dim() != 1 or 2 * frequencies.shape[0] > d:
         raise ValueError("rotary frequencies must be [rotated / 2] with rotated <= D")
     frequencies = _f32_vector("frequencies", frequencies, frequencies.shape[0])
-    at, at_stride = None, 0
+    at, at_stride, wide = None, 0, 0
     if positions is not None:
         positions, at_stride = _token_ints("positions", positions, B, n)
-        at = positions.data_ptr()
+        at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
     q = _rows_contiguous(q)
     q_out = torch.empty_like(q)
     k_out, k_args, k_out_args, G = None, (None, 0, 0, 0), (None, 0, 0, 0), 0
@@ -1038,7 +1038,7 @@ def _rotary(q, k, frequencies, positions, offset, interleaved, magnitude, invers
     args = _capi.RotaryArgs(*_strided(q), *k_args, *_strided(q_out), *k_out_args,
                             frequencies.data_ptr(), at, at_stride, int(offset), B, H, G, n, d,
                             2 * frequencies.shape[0], float(magnitude), code, int(interleaved),
-                            int(inverse))
+                            int(inverse), wide)
     with _on(index):
         _capi.call("xfb_rotary", ctypes.byref(args), _raw_stream(index))
     return q_out, k_out
@@ -1079,9 +1079,9 @@ def _integers(what: str, t: torch.Tensor) -> torch.Tensor:
 
 
 def _token_ints(what: str, t: torch.Tensor, B: int, n: int) -> tuple[torch.Tensor, int]:
-    """int32 [n] or [B, n] with neighbouring tokens next to each other, and its batch stride
-    (0 where one row serves the batch)."""
-    t = _integers(what, t).to(torch.int32)
+    """int32 or int64 [n] or [B, n] with neighbouring tokens next to each other, and its batch
+    stride (0 where one row serves the batch)."""
+    t = _integers(what, t)
     shape = t.shape
     if shape != (B, n) and shape != (n,) and shape != (1, n):
         raise ValueError(f"{what} must be [{n}] or [{B}, {n}], got {list(shape)}")
@@ -1112,14 +1112,15 @@ def _masked_attention_args(q, k, v, scale, softcap, slopes, causal, prefix, docu
     if prefix is not None:
         if prefix.shape != (B,):
             raise ValueError(f"prefix must be [{B}], got {list(prefix.shape)}")
-        prefix = _integers("prefix", prefix)
-        if prefix.dtype != torch.int32:  # no row is longer than 2^30
-            prefix = prefix.clamp(0, 1 << 30)
         prefix = _token_ints("prefix", prefix, 1, B)[0]
+        if prefix.dtype != torch.int32:  # no row is longer than 2^30
+            prefix = prefix.clamp(0, 1 << 30).to(torch.int32)
         prefix_at = prefix.data_ptr()
     if q_doc is not None:
-        q_doc, q_doc_sb = _token_ints("query documents", q_doc, B, nq)
-        k_doc, k_doc_sb = _token_ints("key documents", k_doc, B, nk)
+        q_doc, q_doc_sb = _token_ints("query documents", _integers("query documents", q_doc).to(torch.int32),
+                                     B, nq)
+        k_doc, k_doc_sb = _token_ints("key documents", _integers("key documents", k_doc).to(torch.int32),
+                                     B, nk)
         q_doc_at, k_doc_at = q_doc.data_ptr(), k_doc.data_ptr()
     before = (*_strided(q), *_strided(k), *_strided(v))
     after = (_ptr(slopes), prefix_at, q_doc_at, q_doc_sb, k_doc_at, k_doc_sb, B, H, G, nq, nk, d,
