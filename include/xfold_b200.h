@@ -779,6 +779,14 @@ typedef struct xfb_masked_attention_args {
   void* dv;
   int64_t dv_sb, dv_sh, dv_sn;
 } xfb_masked_attention_args;
+/* Document ids in 64 bits (batch strides q_sb, k_sb; neighbouring tokens next to each other) as the
+ * 32-bit ids that masked attention takes: q_out [batch][nq] and k_out [batch][nk] are equal in a
+ * row where the ids are equal and not negative, and -1 where they are negative. */
+XFB_API int64_t xfb_number_documents_workspace(int64_t batch, int64_t nq, int64_t nk);
+XFB_API int xfb_number_documents(const int64_t* q_ids, int64_t q_sb, int64_t nq,
+                                 const int64_t* k_ids, int64_t k_sb, int64_t nk, int64_t batch,
+                                 int32_t* q_out, int32_t* k_out, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
 /* Bytes that the call with the same arguments needs (pointers and strides included: they
  * choose the kernels). */
 XFB_API int64_t xfb_masked_attention_workspace(const xfb_masked_attention_args* args,

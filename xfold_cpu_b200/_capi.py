@@ -153,6 +153,9 @@ SIGNATURES: dict[str, tuple] = {
     "xfb_layer_norm_backward": (
         _i, [_p, _i64, _p, _i64, _i, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p, _p, _i64, _p]),
     "xfb_rotary": (_i, [_p, _p]),
+    "xfb_number_documents_workspace": (_i64, [_i64, _i64, _i64]),
+    "xfb_number_documents": (
+        _i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
     "xfb_masked_attention_workspace": (_i64, [_p, _i]),
     "xfb_masked_attention": (_i, [_p, _p, _i64, _p]),
     "xfb_masked_attention_backward": (_i, [_p, _p, _i64, _p]),

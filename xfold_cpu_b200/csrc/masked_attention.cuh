@@ -121,6 +121,62 @@ __global__ void __launch_bounds__(256) ma_documents_kernel(MaDocs a) {
   if (lane == 0) a.range[w][b * a.range_sb[w] + range] = make_int4(lo, hi, pad, 0);
 }
 
+// 64-bit ids made 32-bit ones: a document's number is the place of its first token among the
+// row's keys and then its queries, so equal ids keep equal numbers, other ids other ones, and
+// the numbers of documents in order are in order, as the ranges want them.  A hash table of at
+// least twice as many entries as tokens holds (id, first place); only the first token of a
+// run of equal ids enters it, and the least place is the same whatever order they come in.
+struct MaIds {
+  const int64_t* q;
+  const int64_t* k;
+  int64_t q_sb, k_sb;
+  int nq, nk;
+  int32_t* q_out;             // [B][nq]
+  int32_t* k_out;             // [B][nk]
+  unsigned long long* ids;    // [B][2^bits], all ones: empty (no id, ids are not negative)
+  uint32_t* first;            // [B][2^bits], all ones at the start
+  int bits;
+};
+__device__ __forceinline__ int64_t ma_id(const MaIds& a, int b, int64_t at) {
+  return at < a.nk ? a.k[b * a.k_sb + at] : a.q[b * a.q_sb + at - a.nk];
+}
+// The entry of an id: its own, or the first empty one on its way, which ENTER claims.
+template <bool ENTER>
+__device__ __forceinline__ int64_t ma_id_entry(const MaIds& a, int b, int64_t id) {
+  const int64_t size = int64_t(1) << a.bits;
+  unsigned long long* ids = a.ids + b * size;
+  const auto key = static_cast<unsigned long long>(id);
+  // the product's high bits spread neighbouring ids (the multiplier is 2^64 over the golden ratio)
+  int64_t e = static_cast<int64_t>((key * 0x9E3779B97F4A7C15ull) >> (64 - a.bits));
+  for (int64_t tries = 0; tries < size; ++tries, e = (e + 1) & (size - 1)) {
+    const unsigned long long there = ENTER ? atomicCAS(ids + e, ~0ull, key) : ids[e];
+    if (there == key || (ENTER && there == ~0ull)) break;
+  }
+  return b * size + e;
+}
+__global__ void __launch_bounds__(256) ma_ids_enter_kernel(MaIds a) {
+  const int b = blockIdx.y;
+  const int64_t n = int64_t(a.nk) + a.nq;
+  for (int64_t at = blockIdx.x * 256 + threadIdx.x; at < n; at += gridDim.x * 256) {
+    const int64_t id = ma_id(a, b, at);
+    if (id < 0 || (at > 0 && at != a.nk && ma_id(a, b, at - 1) == id)) continue;
+    atomicMin(a.first + ma_id_entry<true>(a, b, id), static_cast<uint32_t>(at));
+  }
+}
+__global__ void __launch_bounds__(256) ma_ids_number_kernel(MaIds a) {
+  const int b = blockIdx.y;
+  const int64_t n = int64_t(a.nk) + a.nq;
+  for (int64_t at = blockIdx.x * 256 + threadIdx.x; at < n; at += gridDim.x * 256) {
+    const int64_t id = ma_id(a, b, at);
+    const int32_t number = id < 0 ? -1 : static_cast<int32_t>(a.first[ma_id_entry<false>(a, b, id)]);
+    if (at < a.nk) {
+      a.k_out[static_cast<int64_t>(b) * a.nk + at] = number;
+    } else {
+      a.q_out[static_cast<int64_t>(b) * a.nq + at - a.nk] = number;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- rows
 
 struct MaRow {

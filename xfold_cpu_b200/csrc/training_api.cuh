@@ -763,6 +763,13 @@ int ma_backward(const xfb::MaskedArgs& m, const MaPlan& p, cudaStream_t st) {
   });
 }
 
+// log2 of the entries of a hash table of n ids: at least twice as many.
+int ma_id_bits(int64_t n) {
+  int bits = 1;
+  while ((int64_t(1) << bits) < 2 * n) ++bits;
+  return bits;
+}
+
 // Sets a strided [B][heads][n][d] tensor to zero.
 template <typename T>
 __global__ void ma_zero_kernel(xfb::MaTensor t, int64_t heads, int64_t n, int64_t d, int64_t total) {
@@ -789,6 +796,40 @@ int ma_zero(const xfb::MaTensor& t, int dtype, int64_t B, int64_t heads, int64_t
 }  // namespace
 
 extern "C" {
+
+XFB_API int64_t xfb_number_documents_workspace(int64_t batch, int64_t nq, int64_t nk) {
+  if (batch <= 0 || nq < 0 || nk < 0 || nq >= (1 << 30) || nk >= (1 << 30) || batch > 65535) return 0;
+  return (batch << ma_id_bits(nq + nk)) * 12;
+}
+
+XFB_API int xfb_number_documents(const int64_t* q_ids, int64_t q_sb, int64_t nq,
+                                 const int64_t* k_ids, int64_t k_sb, int64_t nk, int64_t batch,
+                                 int32_t* q_out, int32_t* k_out, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    XFB_REQUIRE(batch >= 0 && nq >= 0 && nk >= 0, "document sizes must be non-negative");
+    XFB_REQUIRE(batch <= 65535 && nq < (1 << 30) && nk < (1 << 30), "documents are too many");
+    if (batch == 0 || nq + nk == 0) return XFB_OK;
+    XFB_REQUIRE(nq == 0 || (q_ids != nullptr && q_out != nullptr), "documents need query ids");
+    XFB_REQUIRE(nk == 0 || (k_ids != nullptr && k_out != nullptr), "documents need key ids");
+    xfb::MaIds a{q_ids, k_ids, q_sb, k_sb, static_cast<int>(nq), static_cast<int>(nk), q_out, k_out};
+    a.bits = ma_id_bits(nq + nk);
+    const int64_t entries = batch << a.bits;
+    Carver cv{static_cast<uint8_t*>(workspace), entries * 12, workspace_bytes};
+    XFB_TRY(check_workspace(cv, workspace, workspace_bytes));
+    a.ids = static_cast<unsigned long long*>(workspace);
+    a.first = reinterpret_cast<uint32_t*>(a.ids + entries);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    XFB_CUDA(cudaMemsetAsync(workspace, 0xFF, entries * 12, st));
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ceil_div(nq + nk, 256), 4096)),
+                    static_cast<unsigned>(batch));
+    xfb::ma_ids_enter_kernel<<<grid, 256, 0, st>>>(a);
+    XFB_LAUNCHED();
+    xfb::ma_ids_number_kernel<<<grid, 256, 0, st>>>(a);
+    XFB_LAUNCHED();
+    return XFB_OK;
+  });
+}
 
 XFB_API int64_t xfb_masked_attention_workspace(const xfb_masked_attention_args* args,
                                                int backward) {

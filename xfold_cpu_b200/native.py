@@ -1089,6 +1089,28 @@ def _token_ints(what: str, t: torch.Tensor, B: int, n: int) -> tuple[torch.Tenso
     return t, t.stride(0) if t.dim() == 2 and shape[0] > 1 else 0
 
 
+def _number_documents(q, q_sb: int, nq: int, k, k_sb: int, nk: int, B: int, index: int):
+    """int32 ids for document ids of which some are int64, each with its batch stride: the same
+    numbers in a row for the same ids, -1 for negative ones."""
+    same = q is k
+    if k.dtype != torch.int64:
+        k = k.to(torch.int64).contiguous()
+        k_sb = nk if k_sb else 0
+    if q.dtype != torch.int64:
+        q = q.to(torch.int64).contiguous()
+        q_sb = nq if q_sb else 0
+    rows = B if q_sb or k_sb else 1
+    k_out = torch.empty((rows, nk), dtype=torch.int32, device=k.device)
+    q_out = k_out if same else torch.empty((rows, nq), dtype=torch.int32, device=k.device)
+    own = 0 if same else nq
+    with _on(index):
+        ws = _scratch(_capi.load().xfb_number_documents_workspace(rows, own, nk), k)
+        _capi.call("xfb_number_documents", q.data_ptr(), q_sb, own, k.data_ptr(), k_sb, nk, rows,
+                   q_out.data_ptr(), k_out.data_ptr(), _ptr(ws), 0 if ws is None else ws.shape[0],
+                   _raw_stream(index))
+    return q_out, nq if rows > 1 else 0, k_out, nk if rows > 1 else 0
+
+
 _NO_TENSOR = (None, 0, 0, 0)
 
 
@@ -1117,10 +1139,13 @@ def _masked_attention_args(q, k, v, scale, softcap, slopes, causal, prefix, docu
             prefix = prefix.clamp(0, 1 << 30).to(torch.int32)
         prefix_at = prefix.data_ptr()
     if q_doc is not None:
-        q_doc, q_doc_sb = _token_ints("query documents", _integers("query documents", q_doc).to(torch.int32),
-                                     B, nq)
-        k_doc, k_doc_sb = _token_ints("key documents", _integers("key documents", k_doc).to(torch.int32),
-                                     B, nk)
+        same = q_doc is k_doc
+        q_doc, q_doc_sb = _token_ints("query documents", q_doc, B, nq)
+        k_doc, k_doc_sb = (q_doc, q_doc_sb) if same and nq == nk else \
+            _token_ints("key documents", k_doc, B, nk)
+        if q_doc.dtype == torch.int64 or k_doc.dtype == torch.int64:
+            q_doc, q_doc_sb, k_doc, k_doc_sb = _number_documents(q_doc, q_doc_sb, nq, k_doc,
+                                                                 k_doc_sb, nk, B, index)
         q_doc_at, k_doc_at = q_doc.data_ptr(), k_doc.data_ptr()
     before = (*_strided(q), *_strided(k), *_strided(v))
     after = (_ptr(slopes), prefix_at, q_doc_at, q_doc_sb, k_doc_at, k_doc_sb, B, H, G, nq, nk, d,
