@@ -1,0 +1,66 @@
+"""What torch's autograd asks of the differentiable operators beside the gradients' values."""
+
+import pytest
+import torch
+
+from xfold_cpu_b200 import native, training
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda")
+
+
+def tensors(*shape, count=3, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(0)
+    return [torch.randn(*shape, generator=g).to(dtype).to(DEV).requires_grad_()
+            for _ in range(count)]
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("name,mask", [
+    ("documents", lambda: ints(*[0] * 9 + [1] * 11)),
+    ("slopes", lambda: torch.tensor([0.5, 0.25], device=DEV)),
+    ("prefix", lambda: ints(3))])
+def test_a_mask_changed_before_the_backward_pass(name, mask):
+    q, k, v = tensors(1, 2, 20, 16)
+    mask = mask()
+    options = {name: mask, "causal": True}
+    out = training.masked_attention(q, k, v, **options)
+    mask += 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_documents_of_queries_or_keys_changed_before_the_backward_pass(which):
+    q, k, v = tensors(1, 2, 20, 16)
+    documents = ints(*[0] * 20), ints(*[0] * 15 + [1] * 5)
+    out = training.masked_attention(q, k, v, documents=documents)
+    documents[which].fill_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_positions_or_frequencies_changed_before_the_backward_pass(which):
+    q, k = tensors(1, 2, 20, 16, count=2)
+    constants = native.rotary_frequencies(16).to(DEV), torch.arange(20, device=DEV)
+    out = training.rotary(q, k, constants[0], positions=constants[1])
+    constants[which].mul_(2)
+    with pytest.raises(RuntimeError, match="inplace"):
+        (out[0].sum() + out[1].sum()).backward()
+
+
+def test_forms_of_documents_give_the_same_gradients():
+    ids = ints(*[0] * 9 + [1] * 11)
+    grads = []
+    for documents in (ids, ids.long(), (ids, ids), (ids, ids.clone()), [ids, ids.long()]):
+        q, k, v = tensors(1, 2, 20, 16)
+        training.masked_attention(q, k, v, documents=documents, causal=True).sum().backward()
+        grads.append((q.grad, k.grad, v.grad))
+    for other in grads[1:]:
+        for a, b in zip(grads[0], other):
+            assert torch.equal(a, b)

@@ -4,7 +4,7 @@ masked_attention, rotary and layer_norm are the functions of the same names in `
 (layer_norm: layer_norm_forward) with their hand-written backward passes behind
 torch.autograd.Function; linear is a projection on the library's bf16 GEMM with its gradients.
 Their results carry gradients to q, k, v, x, weight and bias; masks, positions, slopes and
-frequencies are constants.  Without gradients (torch.no_grad) nothing is saved.
+frequencies are constants, and must not be changed in place before the backward pass.  Without gradients (torch.no_grad) nothing is saved.
 """
 
 from __future__ import annotations
@@ -14,36 +14,45 @@ import torch
 from . import native
 
 
+def _masks(slopes, prefix, documents, key_documents):
+    """native.masked_attention's masks; without key documents the others serve for both."""
+    return dict(slopes=slopes, prefix=prefix, documents=documents if key_documents is None
+                else (documents, key_documents))
+
+
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, options):
+    def forward(ctx, q, k, v, slopes, prefix, documents, key_documents, options):
+        masks = _masks(slopes, prefix, documents, key_documents)
         if not any(ctx.needs_input_grad):
-            return native.masked_attention(q, k, v, **options)
-        out, (lse, low) = native.masked_attention(q, k, v, save=True, **options)
+            return native.masked_attention(q, k, v, **masks, **options)
+        out, (lse, low) = native.masked_attention(q, k, v, save=True, **masks, **options)
         ctx.options = options
-        ctx.save_for_backward(q, k, v, out, lse, low)
+        # the masks too: the backward pass makes the scores again, and a mask that was changed in
+        # place since would give gradients of another function
+        ctx.save_for_backward(q, k, v, out, lse, low, slopes, prefix, documents, key_documents)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, low = ctx.saved_tensors
+        q, k, v, out, lse, low, *masks = ctx.saved_tensors
         dq, dk, dv = native.masked_attention_backward(dout, q, k, v, out, (lse, low),
-                                                      **ctx.options)
-        return dq, dk, dv, None
+                                                      **_masks(*masks), **ctx.options)
+        return dq, dk, dv, None, None, None, None, None
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, frequencies, options):
-        ctx.save_for_backward(frequencies)
+    def forward(ctx, q, k, frequencies, positions, options):
+        ctx.save_for_backward(frequencies, positions)
         ctx.options = options
-        return native.rotary(q, k, frequencies, **options)
+        return native.rotary(q, k, frequencies, positions=positions, **options)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        frequencies, = ctx.saved_tensors
-        dq, dk = native.rotary_backward(dq, dk, frequencies, **ctx.options)
-        return dq, dk, None, None
+        frequencies, positions = ctx.saved_tensors
+        dq, dk = native.rotary_backward(dq, dk, frequencies, positions=positions, **ctx.options)
+        return dq, dk, None, None, None
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -93,17 +102,19 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                      slopes: torch.Tensor | None = None, causal: bool = False,
                      prefix: torch.Tensor | None = None, documents=None) -> torch.Tensor:
     """native.masked_attention with gradients to q, k and v."""
-    return _MaskedAttention.apply(q, k, v, dict(scale=scale, softcap=softcap, slopes=slopes,
-                                                causal=causal, prefix=prefix,
-                                                documents=documents))
+    key_documents = None
+    if documents is not None and not isinstance(documents, torch.Tensor):
+        documents, key_documents = documents
+    return _MaskedAttention.apply(q, k, v, slopes, prefix, documents, key_documents,
+                                  dict(scale=scale, softcap=softcap, causal=causal))
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, frequencies: torch.Tensor, *,
            positions: torch.Tensor | None = None, offset: int = 0, interleaved: bool = False,
            magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """native.rotary with gradients to q and k."""
-    return _Rotary.apply(q, k, frequencies, dict(positions=positions, offset=offset,
-                                                 interleaved=interleaved, magnitude=magnitude))
+    return _Rotary.apply(q, k, frequencies, positions,
+                         dict(offset=offset, interleaved=interleaved, magnitude=magnitude))
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
