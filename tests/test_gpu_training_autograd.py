@@ -64,3 +64,17 @@ def test_forms_of_documents_give_the_same_gradients():
     for other in grads[1:]:
         for a, b in zip(grads[0], other):
             assert torch.equal(a, b)
+
+
+def test_constants_that_want_a_gradient_are_refused():
+    q, k, v = tensors(1, 2, 20, 16)
+    slopes = torch.tensor([0.5, 0.25], device=DEV, requires_grad=True)
+    frequencies = native.rotary_frequencies(16).to(DEV).requires_grad_()
+    with pytest.raises(RuntimeError, match="slopes"):
+        training.masked_attention(q, k, v, slopes=slopes)
+    with pytest.raises(RuntimeError, match="frequencies"):
+        training.rotary(q, k, frequencies)
+    training.masked_attention(q, k, v, slopes=slopes.detach()).sum().backward()
+    with torch.no_grad():
+        training.masked_attention(q, k, v, slopes=slopes)
+        training.rotary(q, k, frequencies)

@@ -97,11 +97,17 @@ class _Linear(torch.autograd.Function):
         return dx, dw
 
 
+def _constant(what: str, t: torch.Tensor | None) -> None:
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} get no gradient here; pass them detached")
+
+
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                      scale: float | None = None, softcap: float = 0.0,
                      slopes: torch.Tensor | None = None, causal: bool = False,
                      prefix: torch.Tensor | None = None, documents=None) -> torch.Tensor:
     """native.masked_attention with gradients to q, k and v."""
+    _constant("slopes", slopes)
     key_documents = None
     if documents is not None and not isinstance(documents, torch.Tensor):
         documents, key_documents = documents
@@ -113,6 +119,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor, frequencies: torch.Tensor, *,
            positions: torch.Tensor | None = None, offset: int = 0, interleaved: bool = False,
            magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """native.rotary with gradients to q and k."""
+    _constant("frequencies", frequencies)
     return _Rotary.apply(q, k, frequencies, positions,
                          dict(offset=offset, interleaved=interleaved, magnitude=magnitude))
 
