@@ -78,3 +78,25 @@ def test_constants_that_want_a_gradient_are_refused():
     with torch.no_grad():
         training.masked_attention(q, k, v, slopes=slopes)
         training.rotary(q, k, frequencies)
+
+
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_calls_that_need_no_gradient_save_nothing(monkeypatch, grad_mode):
+    """Under no_grad on inputs that require a gradient, and with gradients on for inputs that do
+    not, nothing goes through autograd and the attention keeps no statistics."""
+    calls = []
+    whole = native.masked_attention
+    monkeypatch.setattr(native, "masked_attention",
+                        lambda *a, **o: calls.append(o.get("save", False)) or whole(*a, **o))
+    for name in ("_MaskedAttention", "_Rotary", "_LayerNorm", "_Linear"):
+        monkeypatch.setattr(getattr(training, name), "apply", None)
+    q, k, v = tensors(1, 2, 24, 16)
+    x, w = tensors(24, 16, count=2)
+    frequencies = native.rotary_frequencies(16).to(DEV)
+    if grad_mode:
+        q, k, v, x, w = (t.detach() for t in (q, k, v, x, w))
+    with torch.set_grad_enabled(grad_mode):
+        results = [training.masked_attention(q, k, v), training.layer_norm(x, w[0], w[1]),
+                   training.linear(x, w), *training.rotary(q, k, frequencies)]
+    assert calls == [False]
+    assert not any(t.requires_grad for t in results)

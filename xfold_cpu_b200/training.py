@@ -4,7 +4,8 @@ masked_attention, rotary and layer_norm are the functions of the same names in `
 (layer_norm: layer_norm_forward) with their hand-written backward passes behind
 torch.autograd.Function; linear is a projection on the library's bf16 GEMM with its gradients.
 Their results carry gradients to q, k, v, x, weight and bias; masks, positions, slopes and
-frequencies are constants, and must not be changed in place before the backward pass.  Without gradients (torch.no_grad) nothing is saved.
+frequencies are constants, and must not be changed in place before the backward pass.  Where no
+gradient is wanted (torch.no_grad, or no input requires one) nothing is saved.
 """
 
 from __future__ import annotations
@@ -24,8 +25,6 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, prefix, documents, key_documents, options):
         masks = _masks(slopes, prefix, documents, key_documents)
-        if not any(ctx.needs_input_grad):
-            return native.masked_attention(q, k, v, **masks, **options)
         out, (lse, low) = native.masked_attention(q, k, v, save=True, **masks, **options)
         ctx.options = options
         # the masks too: the backward pass makes the scores again, and a mask that was changed in
@@ -59,9 +58,8 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         y, mean, rstd = native.layer_norm_forward(x, weight, bias, eps)
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(x, weight, mean, rstd)
-            ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
     @staticmethod
@@ -72,11 +70,15 @@ class _LayerNorm(torch.autograd.Function):
                 None if ctx.bias_dtype is None else db.to(ctx.bias_dtype), None)
 
 
+def _linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    return native.linear(x, weight, out_dtype=torch.bfloat16).to(x.dtype)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
         ctx.save_for_backward(x, weight)
-        return native.linear(x, weight, out_dtype=torch.bfloat16).to(x.dtype)
+        return _linear(x, weight)
 
     @staticmethod
     def backward(ctx, dy):
@@ -97,6 +99,11 @@ class _Linear(torch.autograd.Function):
         return dx, dw
 
 
+def _records(*inputs: torch.Tensor | None) -> bool:
+    """Whether autograd is to record a call; inside a Function it cannot be seen any more."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+
+
 def _constant(what: str, t: torch.Tensor | None) -> None:
     if t is not None and t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what} get no gradient here; pass them detached")
@@ -108,6 +115,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                      prefix: torch.Tensor | None = None, documents=None) -> torch.Tensor:
     """native.masked_attention with gradients to q, k and v."""
     _constant("slopes", slopes)
+    if not _records(q, k, v):
+        return native.masked_attention(q, k, v, scale=scale, softcap=softcap, slopes=slopes,
+                                       causal=causal, prefix=prefix, documents=documents)
     key_documents = None
     if documents is not None and not isinstance(documents, torch.Tensor):
         documents, key_documents = documents
@@ -120,6 +130,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor, frequencies: torch.Tensor, *,
            magnitude: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """native.rotary with gradients to q and k."""
     _constant("frequencies", frequencies)
+    if not _records(q, k):
+        return native.rotary(q, k, frequencies, positions=positions, offset=offset,
+                             interleaved=interleaved, magnitude=magnitude)
     return _Rotary.apply(q, k, frequencies, positions,
                          dict(offset=offset, interleaved=interleaved, magnitude=magnitude))
 
@@ -127,9 +140,13 @@ def rotary(q: torch.Tensor, k: torch.Tensor, frequencies: torch.Tensor, *,
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """LayerNorm over the last dimension with gradients to x, weight and bias."""
+    if not _records(x, weight, bias):
+        return native.layer_norm_forward(x, weight, bias, eps)[0]
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """x @ weight^T in bf16 with f32 accumulation (both dimensions of weight multiples of 8)."""
+    if not _records(x, weight):
+        return _linear(x, weight)
     return _Linear.apply(x, weight)
