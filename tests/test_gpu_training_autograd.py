@@ -100,3 +100,19 @@ def test_calls_that_need_no_gradient_save_nothing(monkeypatch, grad_mode):
                    training.linear(x, w), *training.rotary(q, k, frequencies)]
     assert calls == [False]
     assert not any(t.requires_grad for t in results)
+
+
+@pytest.mark.parametrize("call,count", [
+    (lambda a, b: training.linear(a, b), 2),
+    (lambda a, b: training.layer_norm(a, b[0], b[1]), 2),
+    (lambda a, b: training.rotary(a[None, None], b[None, None],
+                                  native.rotary_frequencies(16).to(DEV))[0], 1),
+    (lambda a, b: training.masked_attention(a[None, None], b[None, None], b[None, None]), 2)])
+def test_gradients_of_gradients_are_refused(call, count):
+    """Not left out: what a second backward pass would get through these is missing."""
+    inputs = tensors(24, 16, count=2)
+    w = torch.randn(24, 1, device=DEV).bfloat16().requires_grad_()
+    out = (call(*inputs) * w).float().square().sum()
+    grads = torch.autograd.grad(out, inputs[:count], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        sum(g.float().square().sum() for g in grads).backward()

@@ -5,12 +5,14 @@ masked_attention, rotary and layer_norm are the functions of the same names in `
 torch.autograd.Function; linear is a projection on the library's bf16 GEMM with its gradients.
 Their results carry gradients to q, k, v, x, weight and bias; masks, positions, slopes and
 frequencies are constants, and must not be changed in place before the backward pass.  Where no
-gradient is wanted (torch.no_grad, or no input requires one) nothing is saved.
+gradient is wanted (torch.no_grad, or no input requires one) nothing is saved.  Gradients of
+gradients are refused.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -33,6 +35,7 @@ class _MaskedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, low, *masks = ctx.saved_tensors
         dq, dk, dv = native.masked_attention_backward(dout, q, k, v, out, (lse, low),
@@ -48,6 +51,7 @@ class _Rotary(torch.autograd.Function):
         return native.rotary(q, k, frequencies, positions=positions, **options)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         frequencies, positions = ctx.saved_tensors
         dq, dk = native.rotary_backward(dq, dk, frequencies, positions=positions, **ctx.options)
@@ -63,6 +67,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         dx, dw, db = native.layer_norm_backward(dy, x, weight, mean, rstd)
@@ -81,6 +86,7 @@ class _Linear(torch.autograd.Function):
         return _linear(x, weight)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         n, k = weight.shape
