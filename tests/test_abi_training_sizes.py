@@ -1,4 +1,4 @@
-"""Numbering of 64-bit document ids: argument errors, without a device."""
+"""Argument errors and empty sizes of the training operators' C entry points, without a device."""
 
 import pytest
 
@@ -26,3 +26,11 @@ def test_number_documents_arguments():
     assert call(batch=0) == call(nq=0, nk=0) == _capi.OK
     assert lib.xfb_number_documents_workspace(2, -1, 8) == 0
     assert lib.xfb_number_documents_workspace(0, 4, 8) == 0
+
+
+@pytest.mark.skipif(not LIB_PATH.exists(), reason="library not built")
+def test_linear_of_no_rows():
+    lib = _capi.load()
+    assert lib.xfb_linear(None, 0, 24, 16, 16, None, None, _capi.BF16, 0, None) == _capi.OK
+    assert lib.xfb_linear(None, 0, 20, 16, 16, None, None, _capi.BF16, 0, None) == \
+        _capi.ERR_INVALID

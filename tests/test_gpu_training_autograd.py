@@ -116,3 +116,12 @@ def test_gradients_of_gradients_are_refused(call, count):
     grads = torch.autograd.grad(out, inputs[:count], create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         sum(g.float().square().sum() for g in grads).backward()
+
+
+def test_linear_of_no_rows():
+    w, = tensors(16, 24, count=1)
+    x = torch.zeros(2, 0, 24, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    y = training.linear(x, w)
+    assert y.shape == (2, 0, 16)
+    y.sum().backward()
+    assert x.grad.shape == x.shape and torch.equal(w.grad, torch.zeros_like(w))

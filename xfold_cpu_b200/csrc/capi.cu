@@ -921,6 +921,7 @@ XFB_API int xfb_linear(const void* x, int64_t m, int64_t k, const void* weight, 
   XFB_REQUIRE(y_dtype == XFB_F32 || y_dtype == XFB_BF16, "linear output must be f32 or bf16");
   XFB_REQUIRE(!accumulate || y_dtype == XFB_F32, "accumulate requires an f32 output");
   XFB_REQUIRE(aligned16(y), "linear output must be 16-byte aligned");
+  if (m == 0) return XFB_OK;
   return linear_core(static_cast<const bf16*>(x), m, k, k, static_cast<const bf16*>(weight), n,
                      bias, nullptr, 0, y, y_dtype == XFB_F32, accumulate, n,
                      static_cast<cudaStream_t>(stream));

@@ -94,8 +94,10 @@ class _Linear(torch.autograd.Function):
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = native.linear(dy2, weight.t(), out_dtype=torch.bfloat16).to(x.dtype).view(x.shape)
-        if ctx.needs_input_grad[1]:
-            rows = x2.shape[0]
+        rows = x2.shape[0]
+        if ctx.needs_input_grad[1] and rows == 0:
+            dw = torch.zeros_like(weight)
+        elif ctx.needs_input_grad[1]:
             pad = -rows % 8  # the GEMM reads 16-byte rows along its reduction too
             a, b = dy2.to(torch.bfloat16), x2.to(torch.bfloat16)
             if pad:
