@@ -927,6 +927,14 @@ def _rows_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _empty_rows(t: torch.Tensor) -> torch.Tensor:
+    """An empty result like `t`, its last dimension's values next to each other (empty_like may put
+    those of another dimension there when the rows of `t` overlap)."""
+    r = torch.empty_like(t)
+    return r if r.stride(-1) == 1 or r.shape[-1] <= 1 else \
+        torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _f32_vector(what: str, t: torch.Tensor | None, n: int) -> torch.Tensor | None:
     if t is None:
         return None
@@ -1028,12 +1036,12 @@ def _rotary(q, k, frequencies, positions, offset, interleaved, magnitude, invers
         positions, at_stride = _token_ints("positions", positions, B, n)
         at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
     q = _rows_contiguous(q)
-    q_out = torch.empty_like(q)
+    q_out = _empty_rows(q)
     k_out, k_args, k_out_args, G = None, (None, 0, 0, 0), (None, 0, 0, 0), 0
     if k is not None:
         G = k.shape[1]
         k = _rows_contiguous(_same("k", k, (B, G, n, d), q.dtype))
-        k_out = torch.empty_like(k)
+        k_out = _empty_rows(k)
         k_args, k_out_args = _strided(k), _strided(k_out)
     args = _capi.RotaryArgs(*_strided(q), *k_args, *_strided(q_out), *k_out_args,
                             frequencies.data_ptr(), at, at_stride, int(offset), B, H, G, n, d,
@@ -1178,7 +1186,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     masked_attention_backward takes."""
     index, q, k, v, before, after, held = _masked_attention_args(q, k, v, scale, softcap, slopes,
                                                                  causal, prefix, documents)
-    out = torch.empty_like(q)
+    out = _empty_rows(q)
     lse = low = None
     if save:
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
@@ -1212,7 +1220,7 @@ def masked_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
         low = _contig(_same("saved residual", low, q.shape, torch.bfloat16))
     else:
         low = None
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    dq, dk, dv = _empty_rows(q), _empty_rows(k), _empty_rows(v)
     args = _capi.MaskedAttentionArgs(*before, *_strided(out), lse.data_ptr(), _ptr(low), *after,
                                      *_strided(dout), *_strided(dq), *_strided(dk), *_strided(dv))
     _launch_attention("xfb_masked_attention_backward", 1, args, index, q)
