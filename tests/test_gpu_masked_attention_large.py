@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_masked_attention import DEV, TOL_GRAD, TOL_OUT, close, inputs
+from test_gpu_masked_attention import DEV, TOL_GRAD, TOL_OUT, check, close, inputs
 from xfold_cpu_b200 import _capi, native
 
 pytestmark = pytest.mark.gpu
@@ -105,3 +105,25 @@ def test_every_last_buffer(d, tiles):
     for save in (False, True):
         got = native.masked_attention(q, k, v, save=save)
         close(got[0] if save else got, ref, TOL_OUT[BF16], f"out, save={save}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("softcap", [1e-300, 1e-40, 1e31, 1e38, 1e300])
+def test_caps_that_f32_does_not_hold(dtype, softcap):
+    """A tiny cap makes all scores one, without gradients of q and k; a huge one does nothing."""
+    q, k, v, dout = inputs(1, 4, 2, 150, 150, 64, dtype)
+    check(q, k, v, dout, causal=True, softcap=softcap)
+    if softcap > 1:
+        assert torch.equal(native.masked_attention(q.float(), k.float(), v.float(),
+                                                   softcap=softcap),
+                           native.masked_attention(q.float(), k.float(), v.float())) or \
+            softcap < 2.0 ** 100
+
+
+def test_scales_that_f32_does_not_hold():
+    q, k, v, _ = inputs(1, 2, 2, 20, 20, 16, BF16)
+    for scale in (1e39, -1e300):
+        with pytest.raises(ValueError, match="scale"):
+            native.masked_attention(q, k, v, scale=scale)
+    with pytest.raises(ValueError, match="magnitude"):
+        native.rotary(q, k, native.rotary_frequencies(16).to(DEV), magnitude=1e39)

@@ -320,7 +320,8 @@ XFB_API int xfb_rotary(const xfb_rotary_args* args, void* stream) {
     XFB_REQUIRE(a.d >= 1 && a.d <= 65536, "rotary head dimension must be in [1, 65536]");
     XFB_REQUIRE(a.rotated >= 0 && a.rotated <= a.d && a.rotated % 2 == 0,
                 "rotated dims must be even and at most the head dimension");
-    XFB_REQUIRE(std::isfinite(a.magnitude), "rotary magnitude must be finite");
+    XFB_REQUIRE(std::isfinite(static_cast<float>(a.magnitude)),
+                "rotary magnitude must be finite in f32");
     if (a.batch == 0 || a.n == 0 || a.heads + a.kv_heads == 0) return XFB_OK;
     XFB_REQUIRE(a.heads == 0 || (a.q != nullptr && a.q_out != nullptr), "rotary needs q");
     XFB_REQUIRE(a.kv_heads == 0 || (a.k != nullptr && a.k_out != nullptr), "rotary needs k");
@@ -509,7 +510,7 @@ int ma_check(const xfb_masked_attention_args* args) {
   XFB_REQUIRE(a.heads <= (1 << 20) && a.nk < (1 << 30) &&
                   a.nq * std::max<int64_t>(a.heads / a.kv_heads, 1) < (1 << 30),
               "attention is too long");
-  XFB_REQUIRE(std::isfinite(a.scale), "attention scale must be finite");
+  XFB_REQUIRE(std::isfinite(static_cast<float>(a.scale)), "attention scale must be finite in f32");
   XFB_REQUIRE(std::isfinite(a.softcap) && a.softcap >= 0,
               "attention softcap must be finite and non-negative (0 = none)");
   XFB_REQUIRE(a.prefix == nullptr || a.causal, "a prefix needs causal attention");
@@ -549,8 +550,11 @@ xfb::MaskedArgs ma_args(const xfb_masked_attention_args& a, const MaPlan& p, uin
   m.off = m.nk - m.nq;
   m.causal = a.causal != 0;
   m.scale = static_cast<float>(a.scale);
-  m.cap = static_cast<float>(a.softcap);
-  m.inv_cap = a.softcap > 0 ? static_cast<float>(1.0 / a.softcap) : 0.f;
+  // A cap is held where it and its inverse are normal f32 numbers: below 1e-30 all scores are one
+  // to f32, and above 2^100 no score (2^88 in f32, without an infinity in a product) is bent.
+  const double cap = a.softcap > 0x1p100 ? 0.0 : a.softcap > 0 ? std::max(a.softcap, 1e-30) : 0.0;
+  m.cap = static_cast<float>(cap);
+  m.inv_cap = cap > 0 ? static_cast<float>(1.0 / cap) : 0.f;
   m.q_tiles = p.q_tiles;
   m.k_tiles = p.k_tiles;
   m.splits = p.splits;
