@@ -88,6 +88,8 @@ class PackedAttention(nn.Module):
         """New tokens x [B, n, C] at positions filled, filled + 1, ...: writes their keys and
         values into the cache and attends over what it holds up to them."""
         n = x.shape[1]
+        if filled < 0 or x.shape[0] != cache[0].shape[0]:
+            raise ValueError("filled counts the cache's tokens, and the cache has a row for each of x")
         if filled + n > cache[0].shape[2]:
             raise ValueError("the cache is full")
         q, k, v = self._heads(x, None, filled)
