@@ -748,7 +748,11 @@ XFB_API int xfb_rotary(const xfb_rotary_args* args, void* stream);
  * (bf16 [B][H][nq][d], with bf16 `out` only: what its rounding took away) are what the
  * backward pass needs; NULL: not wanted.
  * The backward pass reads q, k, v, out, lse, out_low (bf16) and dout and writes dq, dk, dv;
- * dk and dv are sums over the query heads that share them. */
+ * dk and dv are sums over the query heads that share them.
+ * bf16 results against one rounding of the exact result: out of a call that wants lse, of few rows
+ * (a new token) or of few row tiles has its error, other calls round the probabilities to bf16
+ * too and have up to 1.4 times it; dq, dk and dv have sqrt(2) times it where nq or nk is above
+ * 512 (probabilities and score gradients rounded to bf16), else its error. */
 typedef struct xfb_masked_attention_args {
   const void* q;
   int64_t q_sb, q_sh, q_sn;

@@ -704,7 +704,7 @@ int ma_forward(const xfb::MaskedArgs& m, const MaPlan& p, cudaStream_t st) {
   return XFB_OK;
 }
 
-// Up to this many queries and keys the backward pass takes P and dX in two parts (eight tiles of 64;
+// In calls of up to this many queries and keys the backward pass takes P and dX in two parts (eight tiles of 64;
 // 2 x 8 heads of 64: 13.8 us in one part and 14.1 in two at 64 tokens, 25.8 and 28.7 at 512).
 constexpr int kMtTwoParts = 512;
 
