@@ -127,3 +127,93 @@ def test_scales_that_f32_does_not_hold():
             native.masked_attention(q, k, v, scale=scale)
     with pytest.raises(ValueError, match="magnitude"):
         native.rotary(q, k, native.rotary_frequencies(16).to(DEV), magnitude=1e39)
+
+
+SLOPES = [2.0 ** (-h / 2 - 1) for h in range(16)]
+
+
+def mask_options(which, B, H, n, qkvo):
+    """Options of a call; documents have padding inside and at the end, which holds NaN."""
+    options = {}
+    if "cap" in which:
+        options["softcap"] = 3.0
+    if "slopes" in which:
+        options["slopes"] = torch.tensor([SLOPES[h % 16] for h in range(H)], device=DEV)
+    if "causal" in which or "prefix" in which:
+        options["causal"] = True
+    if "prefix" in which:
+        options["prefix"] = torch.tensor([n // 2 - 60 * b for b in range(B)], dtype=torch.int32,
+                                         device=DEV)
+    if "documents" in which:
+        g = torch.Generator().manual_seed(9)
+        ids = torch.arange(n).div(n // 3 + 1, rounding_mode="floor").int().repeat(B, 1)
+        ids[torch.rand(B, n, generator=g) < 0.1] = -1
+        ids[:, 70:75], ids[-1, n - 40:] = -1, -1
+        ids = ids.to(DEV)
+        options["documents"] = (ids, ids)
+        for t in qkvo:
+            t.masked_fill_((ids < 0)[:, None, :, None], math.nan)
+    return options
+
+
+MASKS = ["", "causal", "cap", "slopes", "slopes causal", "cap slopes causal", "prefix",
+         "prefix slopes", "cap documents", "slopes causal documents", "causal documents"]
+
+
+@pytest.mark.parametrize("which", MASKS)
+@pytest.mark.parametrize("B,H,G,n,d", [(2, 80, 80, 300, 64), (2, 80, 20, 300, 128),
+                                       (1, 120, 40, 333, 64), (2, 80, 80, 290, 24),
+                                       (1, 150, 150, 259, 128)])
+def test_two_row_tiles_a_block(B, H, G, n, d, which):
+    """One head, four and three (whose tiles have 126 rows) to a K/V head, without the statistics
+    (P in one part) and with them, and the gradients of so many heads."""
+    q, k, v, dout = inputs(B, H, G, n, n, d, BF16)
+    assert two_row_tiles_a_block(q, k)
+    options = mask_options(which, B, H, n, (q, k, v, dout))
+    ref = reference(q, k, v, dout, **options)
+    close(native.masked_attention(q, k, v, **options), ref[0], TOL_OUT[BF16], "out without save")
+    out, saved = native.masked_attention(q, k, v, save=True, **options)
+    close(out, ref[0], TOL_OUT[BF16], "out")
+    grads = native.masked_attention_backward(dout, q, k, v, out, saved, **options)
+    for name, got, want in zip(("dq", "dk", "dv"), grads, ref[1:]):
+        close(got, want, TOL_GRAD[BF16], name)
+
+
+@pytest.mark.parametrize("which", MASKS)
+@pytest.mark.parametrize("B,H,G,n,d", [(1, 4, 4, 1100, 64), (2, 4, 2, 700, 128),
+                                       (1, 6, 2, 601, 128), (1, 8, 1, 530, 48)])
+def test_gradients_in_one_part(B, H, G, n, d, which):
+    """More than 512 tokens: several row and key tiles a block, P and dX rounded once."""
+    q, k, v, dout = inputs(B, H, G, n, n, d, BF16)
+    options = mask_options(which, B, H, n, (q, k, v, dout))
+    ref = reference(q, k, v, dout, **options)
+    out, saved = native.masked_attention(q, k, v, save=True, **options)
+    close(out, ref[0], TOL_OUT[BF16], "out")
+    grads = native.masked_attention_backward(dout, q, k, v, out, saved, **options)
+    for name, got, want in zip(("dq", "dk", "dv"), grads, ref[1:]):
+        close(got, want, TOL_GRAD[BF16], name)
+
+
+@pytest.mark.parametrize("length", [2, 3, 37])
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_short_documents_in_long_rows(length, causal):
+    q, k, v, dout = inputs(1, 4, 2, 1300, 1300, 64, BF16)
+    ids = (torch.arange(1300, device=DEV) // length).int()[None]
+    options = dict(causal=causal, documents=(ids, ids))
+    ref = reference(q, k, v, dout, **options)
+    out, saved = native.masked_attention(q, k, v, save=True, **options)
+    grads = native.masked_attention_backward(dout, q, k, v, out, saved, **options)
+    for name, got, want in zip(("dq", "dk", "dv"), grads, ref[1:]):
+        close(got, want, TOL_GRAD[BF16], name)
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 2000), (5, 700), (700, 90), (130, 1500)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_gradients_in_one_part_of_queries_over_a_cache(nq, nk, d):
+    q, k, v, dout = inputs(2, 8, 2, nq, nk, d, BF16)
+    options = dict(causal=True, softcap=5.0, slopes=torch.tensor(SLOPES[:8], device=DEV))
+    ref = reference(q, k, v, dout, **options)
+    out, saved = native.masked_attention(q, k, v, save=True, **options)
+    grads = native.masked_attention_backward(dout, q, k, v, out, saved, **options)
+    for name, got, want in zip(("dq", "dk", "dv"), grads, ref[1:]):
+        close(got, want, TOL_GRAD[BF16], name)
