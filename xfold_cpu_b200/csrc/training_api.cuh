@@ -529,13 +529,16 @@ bool ma_vec4(const void* p, int64_t sb, int64_t sh, int64_t sn, int size) {
 xfb::MaskedArgs ma_args(const xfb_masked_attention_args& a, const MaPlan& p, uint8_t* ws,
                         bool backward) {
   xfb::MaskedArgs m{};
-  const auto tensor = [](const void* ptr, int64_t sb, int64_t sh, int64_t sn) {
-    return xfb::MaTensor{const_cast<void*>(ptr), sb, sh, sn};
+  // (the stride of a dimension of size one is never used, and may be one that no tensor map takes)
+  const auto tensor = [&a](const void* ptr, int64_t sb, int64_t sh, int64_t sn, int64_t heads,
+                           int64_t n) {
+    return xfb::MaTensor{const_cast<void*>(ptr), a.batch > 1 ? sb : 0, heads > 1 ? sh : 0,
+                         n > 1 ? sn : 0};
   };
-  m.q = tensor(a.q, a.q_sb, a.q_sh, a.q_sn);
-  m.k = tensor(a.k, a.k_sb, a.k_sh, a.k_sn);
-  m.v = tensor(a.v, a.v_sb, a.v_sh, a.v_sn);
-  m.out = tensor(a.out, a.out_sb, a.out_sh, a.out_sn);
+  m.q = tensor(a.q, a.q_sb, a.q_sh, a.q_sn, a.heads, a.nq);
+  m.k = tensor(a.k, a.k_sb, a.k_sh, a.k_sn, a.kv_heads, a.nk);
+  m.v = tensor(a.v, a.v_sb, a.v_sh, a.v_sn, a.kv_heads, a.nk);
+  m.out = tensor(a.out, a.out_sb, a.out_sh, a.out_sn, a.heads, a.nq);
   m.lse = a.lse;
   m.low = static_cast<bf16*>(a.out_low);
   m.slopes = a.slopes;
@@ -577,10 +580,10 @@ xfb::MaskedArgs ma_args(const xfb_masked_attention_args& a, const MaPlan& p, uin
   m.vec4 = a.d % 4 == 0 && ma_vec4(a.q, a.q_sb, a.q_sh, a.q_sn, size) &&
            ma_vec4(a.k, a.k_sb, a.k_sh, a.k_sn, size) && ma_vec4(a.v, a.v_sb, a.v_sh, a.v_sn, size);
   if (backward) {
-    m.dout = tensor(a.dout, a.dout_sb, a.dout_sh, a.dout_sn);
-    m.dq = tensor(a.dq, a.dq_sb, a.dq_sh, a.dq_sn);
-    m.dk = tensor(a.dk, a.dk_sb, a.dk_sh, a.dk_sn);
-    m.dv = tensor(a.dv, a.dv_sb, a.dv_sh, a.dv_sn);
+    m.dout = tensor(a.dout, a.dout_sb, a.dout_sh, a.dout_sn, a.heads, a.nq);
+    m.dq = tensor(a.dq, a.dq_sb, a.dq_sh, a.dq_sn, a.heads, a.nq);
+    m.dk = tensor(a.dk, a.dk_sb, a.dk_sh, a.dk_sn, a.kv_heads, a.nk);
+    m.dv = tensor(a.dv, a.dv_sb, a.dv_sh, a.dv_sn, a.kv_heads, a.nk);
     m.delta = reinterpret_cast<float*>(ws + p.delta);
     m.vec4 = m.vec4 && ma_vec4(a.dout, a.dout_sb, a.dout_sh, a.dout_sn, size);
   }
