@@ -840,8 +840,13 @@ XFB_API int xfb_number_documents(const int64_t* q_ids, int64_t q_sb, int64_t nq,
 
 XFB_API int64_t xfb_masked_attention_workspace(const xfb_masked_attention_args* args,
                                                int backward) {
-  if (ma_check(args) != XFB_OK) return 0;
-  return ma_plan(*args, backward != 0).bytes;
+  int64_t bytes = 0;
+  guarded([&]() -> int {
+    XFB_TRY(ma_check(args));
+    bytes = ma_plan(*args, backward != 0).bytes;
+    return XFB_OK;
+  });
+  return bytes;
 }
 
 XFB_API int xfb_masked_attention(const xfb_masked_attention_args* args, void* workspace,
