@@ -742,8 +742,12 @@ XFB_API int xfb_rotary(const xfb_rotary_args* args, void* stream);
  *   - not causal, or j <= i + nk - nq, or j < prefix[b] (prefix NULL: 0), and
  *   - q_documents[b][i] == k_documents[b][j] >= 0 (both NULL: all one document).
  * A row that sees no key gives zeros; K and V of keys with a negative document never
- * reach a result.  A NaN or infinity of a visible key may also reach rows that do not see
- * it within the same tile of 128 rows and up to 128 keys, as 0 * NaN.
+ * reach a result, nor q and dout of rows that see no key.  A NaN or infinity in any other
+ * key or row may also reach rows and keys that do not see it within the same tile of 128 rows
+ * and up to 128 keys, as 0 * NaN.
+ * Every row of the batch has its queries at the end of its nk keys: several new tokens over rows
+ * filled to different lengths need rows that end together (padding before them, document -1);
+ * one new token does not, as it sees every key that the documents leave.
  * lse (f32 [B][H][nq], natural log of the sum of exp(s); -inf for an empty row) and out_low
  * (bf16 [B][H][nq][d], with bf16 `out` only: what its rounding took away) are what the
  * backward pass needs; NULL: not wanted.

@@ -18,7 +18,7 @@
 // it is the number of tiles in flight that fills the MUFU and the tensor core: two warpgroups
 // and two tiles in flight took 2200 cycles per 2 x 128 x 64 scores at head dim 128.  Measured at
 // 8192 causal tokens, 16 heads on 4: 1030 TFLOP/s at head dim 128, 608 at 64 (softmax
-// instructions: 61 % of the issue slots), 747 and 460 with P in two parts; one token of eight
+// instructions: 56 % of the issue slots), 747 and 460 with P in two parts; one token of eight
 // sequences over 30011 keys 157 us, 5.2 TB/s.
 // The tensor core takes P no wider than bf16 next to bf16 V.  P rounded once puts an error of
 // the size of the result's own rounding on O (2^-9 of the value at most).  Inference over
@@ -839,7 +839,7 @@ __global__ void __launch_bounds__(MtForward<DP, SLOTS_>::kThreads, 1)
 // A tile is 64 wide so that S, dP, two P and dX and two 128-column sums fit the 512 columns.
 // Measured at 8192 causal tokens, 16 heads on 4: dq 1000 TFLOP/s at head dim 128 and 660 at 64 (three
 // products), dk and dv 1130 and 640 (four); bound by the handoffs between a tile's products
-// and its P and dX, with the tensor pipe 50 to 65 % busy.
+// and its P and dX, with the tensor pipe 47 to 59 % busy at 128 and 30 to 32 % at 64.
 
 constexpr int kMtStream = 64;  // streamed rows a tile
 

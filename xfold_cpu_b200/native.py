@@ -1059,7 +1059,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, frequencies: torch.Tensor, *
 
     The first 2 * len(frequencies) dims of each head turn by position * frequency and grow
     by `magnitude`; the others are copied.  Pairs are the halves' (p, p + rotated / 2), or
-    neighbours with `interleaved`.  positions: integers [B, N] or [N]; None: offset + index."""
+    neighbours with `interleaved`.  positions: integers of up to 64 bits, [B, N] or [N]; None:
+    offset + index."""
     return _rotary(q, k, frequencies, positions, offset, interleaved, magnitude, False)
 
 
@@ -1180,7 +1181,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     slopes [H]: s -= slope * |distance|.  causal: keys past the query are hidden, except the
     first prefix[b] (int [B]).  documents: integer ids [B, N] or [N] for Nq = Nk, or a pair
     (query ids, key ids); a query sees keys of its own id only, negative ids (padding)
-    see and are seen by nothing.  A query that sees no key gives zeros.
+    see and are seen by nothing.  A query that sees no key gives zeros.  Ids and prefixes may
+    have 64 bits.
 
     Returns out (q's shape and type), or (out, saved) with save=True: `saved` is what
     masked_attention_backward takes."""
