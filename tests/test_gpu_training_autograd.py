@@ -125,3 +125,17 @@ def test_linear_of_no_rows():
     assert y.shape == (2, 0, 16)
     y.sum().backward()
     assert x.grad.shape == x.shape and torch.equal(w.grad, torch.zeros_like(w))
+
+
+@pytest.mark.parametrize("given", [(True, False), (False, True)])
+def test_documents_of_one_side_are_refused(given):
+    """Not taken for no documents, nor for those of the other side."""
+    q, k, v = tensors(1, 2, 20, 16)
+    documents = tuple(ints(*[0] * 20) if side else None for side in given)
+    for call in (lambda: training.masked_attention(q, k, v, documents=documents),
+                 lambda: native.masked_attention(q.detach(), k.detach(), v.detach(),
+                                                 documents=documents)):
+        with pytest.raises(ValueError, match="documents"):
+            call()
+    assert torch.equal(training.masked_attention(q, k, v, documents=(None, None)),
+                       training.masked_attention(q, k, v))

@@ -1123,11 +1123,19 @@ def _number_documents(q, q_sb: int, nq: int, k, k_sb: int, nk: int, B: int, inde
 _NO_TENSOR = (None, 0, 0, 0)
 
 
+def _document_pair(documents):
+    """(query ids, key ids) of masked attention's `documents`, or (None, None)."""
+    if documents is None or isinstance(documents, torch.Tensor):
+        return documents, documents
+    q_doc, k_doc = documents
+    if (q_doc is None) != (k_doc is None):
+        raise ValueError("documents are given for queries and keys, or for neither")
+    return q_doc, k_doc
+
+
 def _masked_attention_args(q, k, v, scale, softcap, slopes, causal, prefix, documents):
     """(device index, q, k, v, fields before and after the results, tensors they point at)."""
-    if isinstance(documents, torch.Tensor):
-        documents = (documents, documents)
-    q_doc, k_doc = documents if documents is not None else (None, None)
+    q_doc, k_doc = _document_pair(documents)
     index = _train_check(q, k, v, slopes, prefix, q_doc, k_doc)
     code = _train_code(q)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:

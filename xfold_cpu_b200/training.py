@@ -126,9 +126,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     if not _records(q, k, v):
         return native.masked_attention(q, k, v, scale=scale, softcap=softcap, slopes=slopes,
                                        causal=causal, prefix=prefix, documents=documents)
-    key_documents = None
-    if documents is not None and not isinstance(documents, torch.Tensor):
-        documents, key_documents = documents
+    documents, key_documents = native._document_pair(documents)
+    if key_documents is documents:
+        key_documents = None
     return _MaskedAttention.apply(q, k, v, slopes, prefix, documents, key_documents,
                                   dict(scale=scale, softcap=softcap, causal=causal))
 
